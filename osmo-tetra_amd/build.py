@@ -14,6 +14,10 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libtetra_gpu.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
+# no packed FP32 arithmetic: hipcc -O3 makes v_pk_{add,mul,fma}_f32 out of ordinary float code (the phase slicer had six), and some of
+# their forms are not to be relied on; the host pass says that it does not know the feature, which is harmless
+HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 HIP_SRCS = ["tg_k_front.hip", "tg_k_trellis.hip", "tg_k_slot.hip", "tg_k_walk.hip", "tg_k_aux.hip", "tg_cwire.hip", "tg_traffic.hip"]
 C_SRCS = ["tg_host.c", "tg_sync.c", "tg_stream.c", "tg_synth.c", "tg_rm.c", "tg_conv.c", "tg_gsmtap.c", "tg_reorder.c", "tg_comm.c", "tg_stages.c", "tg_cwire.c", "tg_pack.c"]
 HEADERS = ["tg_layout.h", "vit_core.h", "slot_core.h", "tg_internal.h", "tg_dev.h", "tg_dev_vit.h", "tg_conv.h", "tg_cwire.h", "tg_walk_core.h", os.path.join(ROOT, "include", "tetra_gpu.h")]
@@ -53,7 +57,7 @@ def build(force=False, verbose=False):
         if not force and same_flags and not _newer([src] + hdrs + [os.path.abspath(__file__)], o):
             continue
         if s in HIP_SRCS:
-            jobs.append([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall"] + inc + hip_flags + ["-c", src, "-o", o])
+            jobs.append([hipcc] + HIP_FLAGS + inc + hip_flags + ["-c", src, "-o", o])
         else:
             jobs.append(["gcc", "-O3", "-std=gnu11", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter"] + inc + cc_flags +
                         ["-c", src, "-o", o])
