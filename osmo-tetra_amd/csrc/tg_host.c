@@ -1217,7 +1217,8 @@ static int plan_run(struct tgpu_plan *p, const uint8_t *d_stream, uint8_t *d_rec
 	if (fast && p->nslots) {
 		/* blocks that are code words are finished by k_clean; the trellis kernels get the rest, counted on the device */
 		uint32_t *d216 = p->d_dirty + 2, *d432 = d216 + 2 * (size_t)p->max_slots;
-		HCHK(hipMemsetAsync(p->d_dirty, 0, 8, (hipStream_t)stream));
+		if ((rc = tgk_zero16((uint16_t *)p->d_dirty, 4, stream)))
+			return rc;
 		if (fork) {	/* the counters are cleared on the caller's stream: order the side stream behind that */
 			HCHK(hipEventRecord(p->ev_fork, (hipStream_t)stream));
 			HCHK(hipStreamWaitEvent(p->side, p->ev_fork, 0));

@@ -44,6 +44,8 @@ int tgk_slot_t(const uint32_t *d_items, uint32_t nitems, const uint32_t *d_nitem
 	       uint32_t nitems2, const uint32_t *d_nitems2, uint32_t ntotal /* 0, or an upper bound of both lists together */,
 	       const uint32_t *d_packed, const uint32_t *d_masks, const uint32_t *d_maskidx,
 	       uint8_t *d_rec, uint8_t *d_wire /* or NULL */, int flags, void *stream);
+/* n 16-bit words cleared by a kernel (capturable) */
+int tgk_zero16(uint16_t *d, size_t n, void *stream);
 /* clean-block pre-pass (kinds 216 / 432): finishes the blocks that are code words, lists the others for tgk_vit */
 int tgk_clean(int kind, const uint32_t *d_items, uint32_t nitems, const uint32_t *d_packed, const uint32_t *d_masks,
 	      const uint32_t *d_maskidx, uint8_t *d_rec, uint32_t *d_sb_ok, uint32_t *d_sb_code, uint8_t *d_wire,

@@ -1,5 +1,5 @@
 /*
- * tg_k_aux.hip -- tables and init, k_cls_plain, k_reorder, k_fill_*, k_masks, k_grid_*, k_gsmtap, k_stages, the device-walk mid stages
+ * tg_k_aux.hip -- tables and init, k_cls_plain, k_reorder, k_fill_*, k_masks, k_grid_*, k_gsmtap, k_stages, k_zero16, the device-walk mid stages
  * (one of the four HIP units of the library: tg_dev.h has the map)
  */
 #include "tg_dev.h"
@@ -1178,5 +1178,24 @@ extern "C" int tgk_lists2(const uint32_t *d_cls, const uint32_t *d_dbits, uint32
 	hipLaunchKernelGGL(k_lists2, dim3((n + 1024 * TG_MID_CHUNKS - 1) / (1024 * TG_MID_CHUNKS)), dim3(1024), 0, (hipStream_t)stream, d_cls, d_dbits, n, d_okbits, d_prevw,
 			   d_word_chan, d_slot_entry, d_maskidx, d_list_216, d_list_432, d_list_sync ? d_list_all : NULL, d_list_sync, d_cnt, (d_specbits && hints) ? d_specbits : NULL, h, d_chan_code,
 			   d_tbl, nchan);
+	return (int)hipGetLastError();
+}
+
+/* clears n 16-bit words.  A kernel and not a memset of the runtime: the callers' launches may be captured into a graph, and a captured
+ * memset node is not relied on from the second replay on */
+__global__ __launch_bounds__(256)
+void k_zero16(uint16_t *__restrict__ d, size_t n)
+{
+	const size_t step = (size_t)gridDim.x * 256;
+	for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step)
+		d[i] = 0;
+}
+
+extern "C" int tgk_zero16(uint16_t *d, size_t n, void *stream)
+{
+	if (!n)
+		return 0;
+	const size_t blocks = (n + 255) / 256;
+	hipLaunchKernelGGL(k_zero16, dim3((uint32_t)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, (hipStream_t)stream, d, n);
 	return (int)hipGetLastError();
 }

@@ -184,9 +184,8 @@ extern "C" int tgk_traffic(const uint32_t *d_items432, uint32_t n432, const uint
 	if (rc)
 		return rc;
 	hipStream_t s = (hipStream_t)stream;
-	hipError_t e = hipMemsetAsync(d_lens, 0, (size_t)nslots * sizeof(uint16_t), s);
-	if (e != hipSuccess)
-		return (int)e;
+	if ((rc = tgk_zero16(d_lens, nslots, stream)))
+		return rc;
 	const uint32_t items = n432 + n216;
 	if (!items)
 		return 0;
