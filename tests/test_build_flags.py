@@ -1,5 +1,6 @@
-"""The HIP build leaves packed FP32 arithmetic out: checked in the assembly of the one source with vectorisable float code (CPU only,
-the compiler cross-compiles) and in the commands of the recipe."""
+"""The build recipe (CPU only, the compiler cross-compiles): a changed header makes the library stale, the entry point always compiles,
+and packed FP32 arithmetic is left out -- checked in the recipe's commands and in the assembly of the one source with vectorisable
+float code."""
 import importlib.util
 import os
 import re
@@ -44,3 +45,23 @@ def test_float_front_end_has_no_packed_fp32(tmp_path):
     text = open(out).read()
     assert "k_float_to_bits" in text
     assert not re.findall(r"v_pk_(?:add|mul|fma)_f32.*", text)
+
+
+def test_every_included_header_makes_the_library_stale():
+    m = _recipe()
+    named = {os.path.basename(h) for h in m.HEADERS}
+    for f in os.listdir(m.CSRC):
+        for inc in re.findall(r'^#include "(.*?)"', open(os.path.join(m.CSRC, f)).read(), re.M):
+            assert inc in named, (f, inc)
+
+
+def test_entry_point_compiles_also_where_a_library_is_built(monkeypatch):
+    import __graft_entry__ as g
+    import osmo_tetra_amd as T
+    asked = []
+    monkeypatch.setattr(T, "build_library", lambda **kw: asked.append(kw))
+    monkeypatch.setattr(g.subprocess, "check_call", lambda *a, **kw: 0)
+    monkeypatch.setattr(g, "_check_adapter", lambda: None)
+    T.lib()
+    g.build()
+    assert asked == [{"force": True}]
