@@ -20,7 +20,7 @@ HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-X
 
 HIP_SRCS = ["tg_k_front.hip", "tg_k_trellis.hip", "tg_k_slot.hip", "tg_k_walk.hip", "tg_k_aux.hip", "tg_cwire.hip", "tg_traffic.hip"]
 C_SRCS = ["tg_host.c", "tg_sync.c", "tg_stream.c", "tg_synth.c", "tg_rm.c", "tg_conv.c", "tg_gsmtap.c", "tg_reorder.c", "tg_comm.c", "tg_stages.c", "tg_cwire.c", "tg_pack.c"]
-HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".h")) + [os.path.join(ROOT, "include", "tetra_gpu.h")]
+HEADERS = sorted(f for f in (os.listdir(CSRC) if os.path.isdir(CSRC) else []) if f.endswith(".h")) + [os.path.join(ROOT, "include", "tetra_gpu.h")]
 
 
 def _newer(src_list, target):
